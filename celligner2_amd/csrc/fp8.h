@@ -36,6 +36,31 @@ __device__ __forceinline__ unsigned pack8(float a, float b, float c, float d) {
     return (unsigned)r;
 }
 
+// Products with fp32 results run on the bf16 instruction, which adds its products in fp32: every 8-bit number times its scale is
+// exact in bf16.  Eight numbers of FMT (four in lo, four in hi) times the scale `x`, see wide_scale.
+template <int FMT>
+__device__ __forceinline__ bf16x8 widen8(unsigned lo, unsigned hi, float x) {
+    typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
+    bf16x2 a, b, c, d;
+    if (FMT == C2_E4M3) {
+        a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, x, false);
+        b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, x, true);
+        c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, x, false);
+        d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, x, true);
+    } else {
+        a = __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8(lo, x, false);
+        b = __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8(lo, x, true);
+        c = __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8(hi, x, false);
+        d = __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8(hi, x, true);
+    }
+    return bf16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+// The scale byte as the conversion takes it (a float's exponent), one below: a block near fp32's largest number may hold an element
+// that is rounded up to 2^128, which neither fp32 nor bf16 has.  kWideBack times the sum makes up for both operands' halves.  An
+// element under 2^-132 is rounded to a multiple of that (bf16's own smallest step).
+constexpr float kWideBack = 4.f;
+__device__ __forceinline__ float wide_scale(unsigned byte) { return __builtin_bit_cast(float, (byte << 23) - 0x800000u); }
+
 __device__ __forceinline__ int64_t scale_at(int64_t kb, int64_t r64, int64_t row) {
     return ((kb * r64 + (row >> 6)) * 16 + (row & 15)) * 4 + ((row >> 4) & 3);
 }

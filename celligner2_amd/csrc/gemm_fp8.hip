@@ -1,21 +1,25 @@
-// Products of 8-bit block-scaled operands (fp8.hip) on v_mfma_scale_f32_16x16x128_f8f6f4:
+// Products of 8-bit block-scaled operands (fp8.hip):
 //   Y[m][n] = alpha * sum_kb 2^(sA[m][kb] + sB[n][kb]) sum_{k in block kb} A[m][k] B[n][k]  (+ bias[n]),  fp32 accumulation.
 // Forward, input gradient and weight gradient of a Linear layer are this one product (both operands row-wise along the
 // reduction; the quantiser writes the transposed operand where the reduction runs over rows).
 //
-// One block of 128 of the reduction is one instruction: lane l holds 32 bytes of row l % 16, and any assignment of the 128
-// reduction indices to (lane / 16, byte) is right as long as both operands use the same one.  Here a lane takes the 16-byte
-// chunks l / 16 and l / 16 + 4 of its row.
-//
-// What the instruction keeps.  Measured on this chip, and the same for its 16x16x32 and 32x32x64 forms: the products of eight
+// 16-bit results: v_mfma_scale_f32_32x32x64_f8f6f4, two of them to a block of 128 of the reduction.  Lane l holds 32 bytes of row
+// l % 32, and any assignment of the 64 reduction indices to (lane / 32, byte) is right as long as both operands use the same one:
+// in step ks of a block a lane takes the 16-byte chunks 4 ks + 2 (l / 32) and the next one of its row.
+// What that instruction keeps.  Measured on this chip, and the same for its 16x16x32 and 16x16x128 forms: the products of eight
 // neighbours of the reduction are added in fixed point, each cut to a multiple of 2^(E - 13) with E the group's largest sum of
 // exponents; the groups and the accumulator are then added in fp32.  A group of eight is so off by less than 7 * 2^-13 of its
-// largest product (typically 1e-6 to 1e-4 of the result, always towards zero): far below the operands' own 2^-4 / 2^-3, above
-// fp32's.  There is no form without it; a result that needs more is a bf16 product's (c2_linear_fwd).
+// largest product (typically 1e-6 to 1e-4 of the result, always towards zero): far below the operands' own 2^-4 / 2^-3 and a
+// 16-bit result's rounding, above fp32's.
+// fp32 results: the same 32 bytes of a lane, widened in registers (fp8.h), are four v_mfma_f32_32x32x16_bf16, which keep 25 bits
+// below a group's largest product and add the groups and the accumulator in fp32, to nearest (measured: over reductions of 512,
+// 19 200 and 70 400 1e-7, 8e-7 and 1.6e-6 of the result's norm; fp32 arithmetic 1e-7, 6e-7 and 1.3e-6).
 //
 // Bound by the matrix unit where the reduction is long: 8192 x 8192 x 8192 takes 398-411 us, 2.67-2.76 PFLOP/s (the card's
 // library: 2.69).  Short reductions are bound by their results: 4096 x 19 000 over 1024 takes 90-93 us (1.74 PFLOP/s), of which
-// the five rounds' 33 MB of stores, which all CUs make at the same time, are a third.
+// the five rounds' 33 MB of stores, which all CUs make at the same time, are a third.  fp32 results: 8192 cubed 975 us (1.13
+// PFLOP/s, what the library's bf16 product reaches), 1024 x 19 000 over 4096 150 us (88 with a 16-bit result), 4096 x 19 000
+// over 1024 183.
 #include <algorithm>
 
 #include "fp8.h"
@@ -78,7 +82,9 @@ __device__ __forceinline__ f32x16 mma(const i32x8& b, const i32x8& a, const f32x
 // A workgroup walks items (tiles); the stream of loads does not stop between them: the last K-tiles' places ahead hold the
 // next item's first ones, which arrive while the finished tile is stored (B's rows are the matrix unit's rows, so a lane
 // holds neighbouring columns of the result).
-template <int AF, typename TY, int BM, int BN, int WM, int WN, int RA, int RB, int WPE>
+// WIDE (fp32 results; 128 x 128 tiles, since the widened fragments of 256 x 256 do not fit the registers): a row of products is
+// NJ x 4, on fragments of B widened once a step and one of A at a time.
+template <int AF, typename TY, int BM, int BN, int WM, int WN, int RA, int RB, int WPE, bool WIDE>
 __global__ __launch_bounds__(64 * WM * WN, WPE) void gemm_fp8_kernel(Args a, int tiles_m, int tiles_n, int items) {
 #ifdef __HIP_DEVICE_COMPILE__  // (the host pass knows no buffer resources, and drops the kernel's stub over them)
     constexpr int NW = WM * WN, RM = BM / WM, RN = BN / WN, MI = RM / 32, NJ = RN / 32;
@@ -215,10 +221,29 @@ __global__ __launch_bounds__(64 * WM * WN, WPE) void gemm_fp8_kernel(Args a, int
     i32x8 a0[MI], b0[NJ], a1[MI], b1[NJ];
     // one step: NJ x MI products; piece(p) issues a share of the staging loads in front of each row of them
     auto step = [&](const i32x8 (&fa)[MI], const i32x8 (&fb)[NJ], const int (&xa)[SA], const int (&xb)[SB], auto&& piece) {
+        bf16x8 wb[WIDE ? NJ : 1][4];
+        if constexpr (WIDE) {
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) {
+                const float x = wide_scale((unsigned)xb[j / 2] >> (16 * (j & 1)) & 255u);
+#pragma unroll
+                for (int q = 0; q < 4; ++q) wb[j][q] = widen8<C2_E4M3>((unsigned)fb[j][2 * q], (unsigned)fb[j][2 * q + 1], x);
+            }
+        }
 #pragma unroll
         for (int i = 0; i < MI; ++i) {
             piece(i);
             __builtin_amdgcn_sched_barrier(0);
+            if constexpr (WIDE) {
+                const float x = wide_scale((unsigned)xa[i / 2] >> (16 * (i & 1)) & 255u);
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const bf16x8 wa = widen8<AF>((unsigned)fa[i][2 * q], (unsigned)fa[i][2 * q + 1], x);
+#pragma unroll
+                    for (int j = 0; j < NJ; ++j) acc[j][i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(wb[j][q], wa, acc[j][i], 0, 0, 0);
+                }
+                continue;
+            }
 #pragma unroll
             for (int j = 0; j < NJ; ++j) {
                 const int va = xa[i / 2], vb = xb[j / 2];
@@ -326,7 +351,7 @@ __global__ __launch_bounds__(64 * WM * WN, WPE) void gemm_fp8_kernel(Args a, int
         asm volatile("" ::: "memory");
         int ln = lane;  // (opaque: addresses of the stores are formed here, not kept through the loop)
         asm volatile("" : "+v"(ln));
-        const float alpha = a.alpha_dev ? *a.alpha_dev : 1.f;
+        const float alpha = (WIDE ? kWideBack : 1.f) * (a.alpha_dev ? *a.alpha_dev : 1.f);
         const int fa = ra == 0 ? RA - 1 : ra - 1, fb = rb == 0 ? RB - 1 : rb - 1;
         char* strip = (wave < NW / 2 ? ringA + fa * TA : ringB + fb * TB) + (wave & (NW / 2 - 1)) * 32 * SP;
         const int row0 = cur.m0 + wm * RM + ln / 8, col0 = cur.n0 + wn * RN + (ln % 8) * E;
@@ -413,7 +438,7 @@ __global__ __launch_bounds__(256) void join_slabs_kernel(const float* __restrict
         if (n + c < N) st_from_f32<TY>(Y + m * ldy + n + c, alpha * s[c] + (bias ? bias[n + c] : 0.f));
 }
 
-// ---- how a product is cut: tiles of 256 x 256 or 128 x 128, the reduction in `splits` parts where the tiles alone leave CUs
+// ---- how a product is cut (fp32 results: wide): tiles of 256 x 256 or 128 x 128 (wide: these only), the reduction in `splits` parts where the tiles alone leave CUs
 // idle; or 256 x 256 tiles for the columns that make whole rounds of the chip, and the best cut for the rest.
 struct Cut {
     int big, splits, kb_per_split;
@@ -421,25 +446,28 @@ struct Cut {
 };
 // Estimated microseconds, from measurements on random operands: a K-tile takes a 256 x 256 workgroup 1.5 (all CUs busy), two
 // 128 x 128 workgroups on one CU 1.0, a single one 0.9; starting and storing 5 and 4; the join reads its slabs at 5.3 MB/us.
-inline double cost_tiles(bool big, int64_t items, int kb) {
+// Wide: two workgroups 1.7, a single one 1.2; starting and storing 8 and 6 (2048 x 2048 over 1024 and 2048, 256 of them: 17.1 and
+// 26.5; 4096 x 2048, 512: 25.1 and 38.4).
+inline double cost_tiles(bool big, bool wide, int64_t items, int kb) {
+    if (wide) return items <= 256 ? 1.2 * kb + 6. : (double)((items + 511) / 512) * (1.7 * kb + 8.);
     if (big) return (double)((items + 255) / 256) * (1.5 * kb + 5.);
     if (items <= 256) return 0.9 * kb + 4.;
     return (double)((items + 511) / 512) * (1.0 * kb + 4.);
 }
 inline int64_t n_tiles(int64_t n, int e) { return (n + e - 1) / e; }
-inline Cut cut_of(int64_t M, int64_t N, int64_t K, double& least) {
+inline Cut cut_of(int64_t M, int64_t N, int64_t K, bool wide, double& least) {
     const int nkb = (int)n_tiles(K, KB);
     Cut best{};
     best.lds = (N + 3) / 4 * 4;
     best.slab = M * best.lds;
     least = 1e300;
-    for (int big = 0; big < 2; ++big) {
+    for (int big = 0; big < (wide ? 1 : 2); ++big) {
         const int64_t t = big ? n_tiles(M, 256) * n_tiles(N, 256) : n_tiles(M, 128) * n_tiles(N, 128);
         // parts of at least two K-tiles, at most one round of workgroups
         const int64_t most = std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(nkb / 2, 64), (big ? 256 : 512) / t));
         for (int s0 = 1; s0 <= most; ++s0) {
             const int kb = (nkb + s0 - 1) / s0, s = (nkb + kb - 1) / kb;
-            double c = cost_tiles(big, t * s, kb);
+            double c = cost_tiles(big, wide, t * s, kb);
             if (s > 1) c += 3. + (4. * s + 2.) * (double)M * (double)N / 5.3e6;
             if (c < least) {
                 least = c;
@@ -455,31 +483,37 @@ struct Plan {
     int64_t n_big;  // columns of whole rounds of 256 x 256 tiles (0: none)
     Cut cut;        // of the rest
 };
-inline Plan plan_of(int64_t M, int64_t N, int64_t K) {
+inline Plan plan_of(int64_t M, int64_t N, int64_t K, bool wide) {
     double whole, rest;
-    Plan p{0, cut_of(M, N, K, whole)};
+    Plan p{0, cut_of(M, N, K, wide, whole)};
+    if (wide) return p;
     const int64_t tm = n_tiles(M, 256), full = tm * n_tiles(N, 256) / 256 * 256 / tm * 256;
     if (full > 0 && full < N) {
-        const Cut r = cut_of(M, N - full, K, rest);
-        if (cost_tiles(true, tm * (full / 256), (int)n_tiles(K, KB)) + rest < whole) p = {full, r};
+        const Cut r = cut_of(M, N - full, K, false, rest);
+        if (cost_tiles(true, false, tm * (full / 256), (int)n_tiles(K, KB)) + rest < whole) p = {full, r};
     }
     return p;
 }
 
-template <int AF, typename TY>
+template <int AF, typename TY, bool WIDE>
 void launch_tiles(const Args& a, const Cut& c, hipStream_t st) {
 #define TILE(BM, BN, WM, WN, PER_CU)                                                                                       \
     do {                                                                                                                   \
         const int tm = (int)n_tiles(a.M, BM), tn = (int)n_tiles(a.N, BN), items = tm * tn * c.splits;                      \
         /* a walk over several items: the loads run two K-tiles ahead, into the next item but not past it */               \
         const int grid = c.splits == 1 && a.nkb >= 2 ? std::min(items, 256 * PER_CU) : items;                              \
-        auto k = gemm_fp8_kernel<AF, TY, BM, BN, WM, WN, 3, 2, 2>;                                                         \
+        auto k = gemm_fp8_kernel<AF, TY, BM, BN, WM, WN, 3, 2, 2, WIDE>;                                                       \
         constexpr int lds = (3 * BM + 2 * BN) * KB;                                                                        \
         (void)hipFuncSetAttribute((const void*)k, hipFuncAttributeMaxDynamicSharedMemorySize, lds);                        \
         hipLaunchKernelGGL(k, dim3((unsigned)grid), dim3(64 * WM * WN), lds, st, a, tm, tn, items);                        \
     } while (0)
-    if (c.big) TILE(256, 256, 2, 4, 1);
-    else TILE(128, 128, 2, 2, 2);
+    if constexpr (!WIDE) {
+        if (c.big) {
+            TILE(256, 256, 2, 4, 1);
+            return;
+        }
+    }
+    TILE(128, 128, 2, 2, 2);
 #undef TILE
 }
 
@@ -505,6 +539,7 @@ void join_slabs(const float* ws, int64_t slab, int64_t lds, int splits, int64_t 
 
 template <typename TY>
 void launch(const Args& a0, const Cut& c, int a_fmt, float* ws, hipStream_t st) {
+    constexpr bool WIDE = sizeof(TY) == 4;  // (the parts of a 16-bit result are what its own form makes)
     Args a = a0;
     a.kb_per_split = c.kb_per_split;
     if (c.splits > 1) {
@@ -513,13 +548,13 @@ void launch(const Args& a0, const Cut& c, int a_fmt, float* ws, hipStream_t st) 
         a.slab = c.slab;
         a.bias = nullptr;
         a.alpha_dev = nullptr;
-        if (a_fmt == C2_E4M3) launch_tiles<0, float>(a, c, st);
-        else launch_tiles<1, float>(a, c, st);
+        if (a_fmt == C2_E4M3) launch_tiles<0, float, WIDE>(a, c, st);
+        else launch_tiles<1, float, WIDE>(a, c, st);
         join_to<TY>(ws, c.slab, c.lds, c.splits, a0.M, a0.N, (TY*)a0.Y, a0.ldy, a0.bias, a0.alpha_dev, st);
         return;
     }
-    if (a_fmt == C2_E4M3) launch_tiles<0, TY>(a, c, st);
-    else launch_tiles<1, TY>(a, c, st);
+    if (a_fmt == C2_E4M3) launch_tiles<0, TY, WIDE>(a, c, st);
+    else launch_tiles<1, TY, WIDE>(a, c, st);
 }
 
 template <typename TY>
@@ -540,7 +575,7 @@ void product_to(Args a, const Plan& p, int a_fmt, float* ws, hipStream_t st) {
 void product(const void* A, int64_t lda, const uint8_t* sA, int a_fmt, const void* B, int64_t ldb, const uint8_t* sB, int64_t M,
              int64_t N, int64_t K, void* Y, int y_dtype, int64_t ldy, const float* bias, const float* alpha_dev, float* ws,
              hipStream_t st) {
-    const Plan p = plan_of(M, N, K);
+    const Plan p = plan_of(M, N, K, y_dtype == C2_F32);
     Args a{(const uint8_t*)A, (const uint8_t*)B, (const uint32_t*)sA, (const uint32_t*)sB, Y, bias, alpha_dev,
            lda, ldb, ldy, 0, (int)M, (int)N, (int)n_tiles(K, KB), 0, (int)n_tiles(M, 64), (int)n_tiles(N, 64), 0};
     if (y_dtype == C2_F32) product_to<float>(a, p, a_fmt, ws, st);
@@ -552,8 +587,12 @@ size_t product_ws(int64_t M, int64_t N, int64_t K) {
         const RowPlan r = row_plan(M, N, K);
         return r.splits > 1 ? (size_t)r.splits * (size_t)M * (size_t)r.lds : 0;
     }
-    const Plan p = plan_of(M, N, K);
-    return p.cut.splits > 1 ? (size_t)p.cut.splits * (size_t)p.cut.slab : 0;
+    size_t floats = 0;  // whatever the result's type
+    for (const bool wide : {false, true}) {
+        const Cut c = plan_of(M, N, K, wide).cut;
+        if (c.splits > 1) floats = std::max(floats, (size_t)c.splits * (size_t)c.slab);
+    }
+    return floats;
 }
 
 // bytes of x's 8-bit copy and its scales in the workspace of c2_linear_fwd_fp8, each on 16 bytes

@@ -586,7 +586,8 @@ def _forward_fp8(x, w, y, out_dtype, bias, ws):
 
 
 def linear_fwd_fp8(x, w, y=None, bias=None, out_dtype=torch.bfloat16, ws=None):
-    """y = x @ w.T (+ bias) on 8-bit operands.  x [M, K]: Fp8Blocks, or a fp32 / bf16 / half matrix, quantised here to e4m3;
+    """y = x @ w.T (+ bias) on 8-bit operands (a fp32 result has fp32 accuracy, at about half the speed of a 16-bit one, which keeps
+    13 bits of each eight products: include/c2mi.h, c2_linear_fp8).  x [M, K]: Fp8Blocks, or a fp32 / bf16 / half matrix, quantised here to e4m3;
     w [N, K]: Fp8Blocks (quant_fp8(weight, block_rows=128)).  y: [M, N] of out_dtype, made when None.  Few, short rows of x (a
     served query: M <= 16 and M * ceil(K / 128) <= 64) are quantised and multiplied in one launch.  ws: a contiguous tensor of
     4 * linear_fp8_ws(M, N, K) bytes for quantised x, linear_fwd_fp8_ws(M, N, K) bytes else; taken from torch's allocator when
