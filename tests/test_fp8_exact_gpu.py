@@ -1,6 +1,10 @@
-"""fp32 results of 8-bit products have fp32 accuracy.
+"""8-bit products where every bit is known, and fp32 results to fp32 accuracy.
 
-Their products are exact, the matrix unit adds eight neighbours with 25 bits below the largest, cutting each (an
+Known operands.  Entries +-2^e with one e (-1, 0 or 1) for each row and block of 128: every block quantises exactly, products within a
+block have one exponent, so the matrix unit's groups lose nothing, and sums are multiples of 1/4 below 4 K < 2^22: exact in fp32
+in any order.  A term left out, taken twice or with a neighbour's scale shows in torch.equal.
+
+fp32 results.  Their products are exact, the matrix unit adds eight neighbours with 25 bits below the largest, cutting each (an
 error under 7 * 2^-25 of the largest), and groups and accumulator in fp32: K / 8 + 16 additions and a few for joined parts, bias
 and alpha.  (1) Element by element those errors add up to less than 7 * 2^-25 * sum of the groups' largest + n 2^-24 sum |a||b|.
 (2) Roundings are independent of each other and of the signs here, so over a whole result their squares add up: each is at most
@@ -15,6 +19,7 @@ from tests.test_fp8_gpu import SHAPES, _matrix
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
+DT = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
 
 
 def _ops():
@@ -22,8 +27,56 @@ def _ops():
     return ops
 
 
+def _signs(R, C, seed, rows=1):
+    """+-2^e, one e for `rows` rows and 128 columns, fp32 on the device."""
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    e = torch.randint(-1, 2, (-(-R // rows), -(-C // 128)), generator=g, device=DEV).float()
+    e = e.repeat_interleave(rows, 0)[:R].repeat_interleave(128, 1)[:, :C]
+    return (torch.randint(0, 2, (R, C), generator=g, device=DEV).float() * 2 - 1) * torch.exp2(e)
+
+
 def _exact(a, b):
     return torch.mm(a.double(), b.double().t().contiguous())
+
+
+def _same(y, ref):
+    want = ref.to(torch.float32).to(y.dtype)
+    assert torch.equal(y, want), (y.dtype, (y != want).sum().item(), (y != want).nonzero()[0].tolist())
+
+
+@pytest.mark.parametrize("M,N,K", SHAPES + [(64, 300, 70000), (128, 256, 19000), (100, 300, 12000), (300, 19001, 130)])
+def test_every_term_counts_once(M, N, K):
+    ops = _ops()
+    x, w, w1 = _signs(M, K, M + K), _signs(N, K, N + K, 128), _signs(N, K, N + K + 1)
+    bias = torch.randint(-9, 10, (N,), device=DEV).float()
+    alpha = torch.tensor([0.5], device=DEV)
+    ref, ref1 = _exact(x, w), _exact(x, w1)
+    wq, w1q, xq, x5 = ops.quant_fp8(w, block_rows=128), ops.quant_fp8(w1), ops.quant_fp8(x), ops.quant_fp8(x, fmt="e5m2")
+    for dt in DT.values():
+        _same(ops.linear_fwd_fp8(x, wq, bias=bias, out_dtype=dt), ref + bias.double())
+        _same(ops.linear_fwd_fp8(x.bfloat16(), w1q, out_dtype=dt), ref1)
+        _same(ops.linear_fwd_fp8(xq, wq, out_dtype=dt), ref)
+        _same(ops.linear_dgrad_fp8(x5, w1q, alpha=alpha, out_dtype=dt), ref1 * 0.5)
+
+
+# How these are cut for 16-bit results: 256 x 256 tiles in four parts of the reduction; whole rounds of them for 16 384 columns and
+# the rest in three parts; whole rounds and a rest that is not cut, ragged at every edge; 256 x 256 tiles alone.  `floats`: the
+# workspace of that cut (fp32 results take fewer parts here), so that another cut shows.
+@pytest.mark.parametrize("M,N,K,floats", [(1024, 4096, 8192, 4 * 1024 * 4096), (1024, 19000, 4096, 3 * 1024 * 2616),
+                                          (777, 19001, 820, None), (4096, 4096, 300, 0)])
+def test_large_cuts(M, N, K, floats):
+    ops = _ops()
+    if floats is not None:
+        assert ops.linear_fp8_ws(M, N, K) == floats
+    x, w = _signs(M, K, 1), _signs(N, K, 2)
+    ref = _exact(x, w)
+    bias = torch.randint(-9, 10, (N,), device=DEV).float()
+    alpha = torch.tensor([0.25], device=DEV)
+    wq = ops.quant_fp8(w)
+    for dt in (torch.bfloat16, torch.float32, torch.float16):
+        _same(ops.linear_fwd_fp8(ops.quant_fp8(x), wq, bias=bias, out_dtype=dt), ref + bias.double())
+        for fmt in ("e4m3", "e5m2"):
+            _same(ops.linear_dgrad_fp8(ops.quant_fp8(x, fmt=fmt), wq, alpha=alpha, out_dtype=dt), ref * 0.25)
 
 
 def _fp32_result(y, a, b, extra=None):
