@@ -5,8 +5,9 @@
 //   over its whole vocabulary is given (then P = sum_k p_k <= 1; else P = 1)
 //   loss   = T^2 c sum_b w_b sum_k p_k (log p_k - log q_{i_k})
 //   ds_j   = T c w_b (P q_j - sum_{k: i_k = j} p_k),   c = inv_B
-// With e_k = exp(t_k/T - mT), z = sum e_k (or z = 1 and mT = lse): p_k = e_k / z, and the row's sum over the list is
-//   (U - W) / z - P log z + P log Z,  U = sum e_k (t_k/T - mT),  W = sum e_k (s_{i_k} - mS)/T,  Z = sum_j exp((s_j - mS)/T),
+// With e_k = exp(d_k), d_k = (t_k - max t) / T (of the logits' difference: t / T itself may be large, and its rounding with it) and
+// z = sum e_k, or d_k = t_k / T - lse and z = 1: p_k = e_k / z, and the row's sum over the list is
+//   (U - W) / z - P log z + P log Z,  U = sum e_k d_k,  W = sum e_k (s_{i_k} - mS)/T,  Z = sum_j exp((s_j - mS)/T),
 // so that every sum of the row (Z, z, U, W) is formed after the two maxima and one more reduction ends the row.
 //
 // Bound by memory: a row is read once and its gradient written once (311 MB at 4096 x 19 000 in bf16: 69-71 us, 4.5 TB/s, 0.88 of
@@ -89,16 +90,21 @@ __device__ __forceinline__ void row_reduce(float (&v)[N], float* red) {
     }
 }
 
-// A teacher's logit / T in the list's maximum: a NaN as infinity, so that a row whose logits are all NaN is not taken for one
+// A teacher's logit in the list's maximum: a NaN as infinity, so that a row whose logits are all NaN is not taken for one
 // without a list (the exponentials of the others are then zero, its own NaN).
 __device__ __forceinline__ float in_max(float x) { return x == x ? x : INFINITY; }
 
-// The list of row b into LDS (index -1: absent) and its largest logit / T; t, nt: the row's threads.
+// log e of a list entry (above); mt: the list's largest logit, or the teacher's normaliser
+__device__ __forceinline__ float list_arg(const Args& a, float x, float mt) {
+    return a.lse ? fmaf(x, a.it, -mt) : (x - mt) * a.it;
+}
+
+// The list of row b into LDS (index -1: absent) and its largest logit; t, nt: the row's threads.
 __device__ __forceinline__ float load_list(const Args& a, int64_t b, int t, int nt, int* lidx, float* lval, bool report) {
     float mt = -INFINITY;
     for (int k = t; k < a.K; k += nt) {
         const int64_t i = list_index(a, b, k);
-        const float v = a.top[b * a.ldt + k] * a.it;
+        const float v = a.top[b * a.ldt + k];
         const bool on = i >= 0 && i < a.V;
         if (report && i >= a.V && a.status) *a.status = 1;
         lidx[k] = on ? (int)i : -1;
@@ -231,7 +237,7 @@ __global__ __launch_bounds__(64 * W * RPB) void distill_row_kernel(Args a) {
             }
         }
         li = join_index(a, lilo, lihi);
-        tv = ltop * a.it;
+        tv = ltop;
         rw = a.weight ? w : 1.f;
         rlse = lse;
     };
@@ -259,7 +265,7 @@ __global__ __launch_bounds__(64 * W * RPB) void distill_row_kernel(Args a) {
         }
         for (int k = t + NT; k < a.K; k += NT) {
             const int64_t i = list_index(a, b, k);
-            const float x = a.top[b * a.ldt + k] * a.it;
+            const float x = a.top[b * a.ldt + k];
             const bool o = i >= 0 && i < a.V;
             if (i >= a.V && a.status) *a.status = 1;
             lidx[k] = o ? (int)i : -1;
@@ -280,7 +286,7 @@ __global__ __launch_bounds__(64 * W * RPB) void distill_row_kernel(Args a) {
                 const int j = lidx[k];
                 if (j < 0) continue;
                 add_named(named, j);
-                const float d = lval[k] - mt, e = expf(d), u = (k == t ? sj : load1(s + j)) - ms;
+                const float d = list_arg(a, lval[k], mt), e = expf(d), u = (k == t ? sj : load1(s + j)) - ms;
                 if (!(e == 0.f)) {  // (0 * infinity where a class is impossible on both sides)
                     r[1] += e;
                     r[2] += e * d;
@@ -427,7 +433,7 @@ __global__ __launch_bounds__(256) void distill_seg_grad_kernel(Args a, int64_t n
     for (int k = t; k < a.K; k += 256) {
         if (lidx[k] < 0) continue;
         add_named(named, lidx[k]);
-        const float d = lval[k] - mt, e = expf(d), u = seg_listed(a, nseg, b)[k] - ms;
+        const float d = list_arg(a, lval[k], mt), e = expf(d), u = seg_listed(a, nseg, b)[k] - ms;
         if (!(e == 0.f)) {
             r[1] += e;
             r[2] += e * d;
