@@ -357,8 +357,8 @@ int c2_classifier_loss_fwd_bwd(const float* u, int64_t ldu, int64_t* classes, in
 
 /* Distillation from a teacher's top logits, forward and backward (no counterpart in the reference; a query model tuned by
  * surgery is kept near its reference model's strongest genes or labels).  Row b: student logits over V classes, the teacher's
- * list (top_idx, top_logits)[b][0..K), K <= 1024 (idx_bytes 4: int32, 8: int64; row pitches ldi, ldt), temperature T > 0
- * (1 / T and T^2 finite):
+ * list (top_idx, top_logits)[b][0..K), K <= 1024 (idx_bytes 4: int32, 8: int64; row pitches ldi, ldt), temperature T from 1.1e-19
+ * to 1.8e19 (T^2 a normal fp32 number):
  *   q = softmax(s / T);  p = softmax over the list of t / T, or exp(t / T - teacher_lse[b]) when teacher_lse [B] is given (the
  *   log of the teacher's normaliser sum exp(t / T) over its whole vocabulary);
  *   loss_out = T^2 inv_B sum_b weight[b] sum_k p_k (log p_k - log q_k)     (added to loss_out when loss_add);

@@ -42,3 +42,10 @@ def test_embed_entries_refuse():
                 dict(D=(1 << 23) + 1, ldd=1 << 24, ldt=1 << 24), dict(N=200, ws=None), dict(N=200, ws=P + 4), dict(d=None), dict(ids=None), dict(o=None), dict(ldd=7), dict(ldt=7)):
         assert grad(**bad) != 0, bad
     assert grad(V=0) == 0 and grad(D=0) == 0
+
+
+@pytest.mark.parametrize("T", [1e-19, 1e-20, 1e-23, 3e-39, 4e-39])
+def test_temperatures_whose_square_is_not_a_normal_number_are_refused(T):
+    """T^2 scales the loss: at 1e-20 it keeps a few bits, at 1e-23 it is zero; at 3e-39 log2(e) / T is infinite."""
+    rc = lib.c2_distill_topk_fwd_bwd(P, 0, 50, P, 8, 3, P, 3, 3, None, None, T, 4, 50, 1.0, P, 1, P + 64, 0, 50, P, None, None)
+    assert rc != 0 and b"temperature" in lib.c2_last_error()
