@@ -451,11 +451,15 @@ __device__ __forceinline__ void add_parts(const Sum& a, int64_t c, int first, in
     }
 }
 
+// (added to what is there: a sum of zero leaves it as it is, bit for bit -- that of a row without a token in few_rows_join_kernel)
 __device__ __forceinline__ void write_row4(const Sum& a, int v, int64_t c, f32x4 s) {
     float* row = a.dtable + (int64_t)v * a.ldt;
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-        if (c + j < a.D) row[c + j] = a.accumulate ? row[c + j] + s[j] * a.scale : s[j] * a.scale;
+    for (int j = 0; j < 4; ++j) {
+        if (c + j >= a.D) continue;
+        if (!a.accumulate) row[c + j] = s[j] * a.scale;
+        else if (s[j] != 0.f) row[c + j] += s[j] * a.scale;
+    }
 }
 
 __global__ __launch_bounds__(1024) void join_kernel(Sum a) {
