@@ -810,6 +810,7 @@ extern "C" int c2_embed_grad(const void* dout, int d_dtype, int64_t ldd, const v
     C2_CHECK(V >= 0 && D >= 0 && N >= 0 && N <= (1ll << 26) && V <= (1ll << 27) && D <= (1ll << 23), "bad shape");
     C2_CHECK(d_dtype == C2_F32 || d_dtype == C2_BF16 || d_dtype == C2_F16, "bad gradient dtype");
     C2_CHECK(idx_bytes == 4 || idx_bytes == 8, "idx_bytes: 4 (int32) or 8 (int64)");
+    C2_CHECK(scale - scale == 0.f, "scale must be finite");  // (rows without a token are sums of zero, scaled, in some forms)
     if (V == 0 || D == 0) return 0;
     C2_CHECK(dtable && ldt >= D && (N == 0 || (dout && ids && ldd >= D)), "bad arguments");
     C2_CHECK(c2_embed_grad_ws(N, V, D) == 0 || (ws && aligned16(ws)), "workspace: null, or not on 16 bytes");

@@ -1009,7 +1009,7 @@ def embed_grad_ws(N, V, D):
 
 
 def embed_grad(dout, ids, V, scale=1.0, dtable=None, accumulate=False, status=None, ws=None):
-    """dtable[v] = scale * sum of dout[n] over the tokens with ids[n] = v, fp32 [V, D] (made when None); accumulate: added to
+    """dtable[v] = scale (finite) * sum of dout[n] over the tokens with ids[n] = v, fp32 [V, D] (made when None); accumulate: added to
     dtable, rows without a token untouched.  dout [N, D] fp32 / bf16 / half; ids and status as in embed_fwd.  ws: a
     contiguous tensor of embed_grad_ws(N, V, D) bytes, made when None."""
     dev = _device(dout, ids, dtable, status, ws)

@@ -368,7 +368,8 @@ int c2_classifier_loss_fwd_bwd(const float* u, int64_t ldu, int64_t* classes, in
  * logits are.  An index >= V is left out and sets *status_dev (may be NULL) to 1.  A class with s = -infinity has q = 0; one
  * that the teacher lists with p > 0 makes the loss infinite.  A NaN in a row that counts makes the loss and its row NaN.
  * logits fp32, bf16 or half; dlogits fp32 or bf16, NULL (loss only), or the logits themselves (same type and pitch); it must
- * not overlap them otherwise.
+ * not overlap them otherwise.  Without rows or classes (B or V zero) nothing is launched and the status word is left.  Rows of more
+ * than 32 768 classes: fewer than 2^24 pieces of 8192 classes in all.
  * ws: c2_distill_topk_ws(B, V, K) floats.  The loss's second stage is subject to c2_defer_loss_sums. */
 size_t c2_distill_topk_ws(int64_t B, int64_t V, int K);
 int c2_distill_topk_fwd_bwd(const void* logits, int l_dtype, int64_t ldl, const void* top_idx, int idx_bytes, int64_t ldi,
@@ -488,7 +489,8 @@ int c2_gather_rows_ld(const float* X, int64_t ldX, const uint8_t* goodloc, int64
  *                  written (rows without a token: zero, or left as they are when accumulate); dout [N, D] fp32 / bf16 / half
  * ids [N]: idx_bytes 4 (int32) or 8 (int64).  A negative id is a place without a token: a zero row, no gradient; an id >= V
  * too, and sets *status_dev (may be NULL) to 1.  Sums in fp32 in an order fixed by the ids: the same bits on every call.
- * ws: c2_embed_grad_ws(N, V, D) bytes, 16-byte aligned.  N <= 2^26 tokens, V <= 2^27, D <= 2^23. */
+ * ws: c2_embed_grad_ws(N, V, D) bytes, 16-byte aligned.  N <= 2^26 tokens, V <= 2^27, D <= 2^23; the gradient's scale is
+ * finite.  A call with nothing to write (a size of zero) launches nothing and leaves the status word. */
 int c2_embed_fwd(const void* table, int t_dtype, int64_t ldt, int64_t V, int64_t D, const void* ids, int idx_bytes, int64_t N,
                  float scale, void* out, int out_dtype, int64_t ldo, int32_t* status_dev, void* stream);
 size_t c2_embed_grad_ws(int64_t N, int64_t V, int64_t D);

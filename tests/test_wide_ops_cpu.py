@@ -49,3 +49,9 @@ def test_temperatures_whose_square_is_not_a_normal_number_are_refused(T):
     """T^2 scales the loss: at 1e-20 it keeps a few bits, at 1e-23 it is zero; at 3e-39 log2(e) / T is infinite."""
     rc = lib.c2_distill_topk_fwd_bwd(P, 0, 50, P, 8, 3, P, 3, 3, None, None, T, 4, 50, 1.0, P, 1, P + 64, 0, 50, P, None, None)
     assert rc != 0 and b"temperature" in lib.c2_last_error()
+
+
+@pytest.mark.parametrize("scale", [float("inf"), float("-inf"), float("nan")])
+def test_gradient_scales_that_are_not_finite_are_refused(scale):
+    """A row without a token is zero, not 0 * scale."""
+    assert lib.c2_embed_grad(P, 0, 8, P, 4, 3, 5, 8, scale, P, 8, 0, P, None, None) != 0 and b"finite" in lib.c2_last_error()
