@@ -4,11 +4,13 @@
 // reported through the status word.
 //
 // Lookup: bound by memory.  A thread moves 8 neighbouring columns of four rows, the four ids fetched together, then the four
-// pieces of the table, then the stores.  65 536 tokens of 512 columns in bf16: 14.8 us, 4.5 TB/s of rows written (the table,
-// 19 MB, comes from the caches); 128 tokens of 128: 2.6 us.
+// pieces of the table, then the stores.  65 536 tokens of 512 columns in bf16: 17.0 us (at best 14.5), 67 MB of rows written at 4.0
+// TB/s (the table, 19 MB, comes from the caches); 128 tokens of 128: 3.0 us.
 //
 // Gradient: the tokens are put in the order of their ids (a stable radix sort of 8 bits a pass), and the sorted list is cut
-// into chunks of equal length, whatever the ids: a row that half of the tokens read costs no more than as many different rows.
+// into chunks of equal length, whatever the ids: a row that half of the tokens read costs the sums no more than as many different
+// rows (its parts, one a chunk, are joined by one workgroup for 256 columns: 65 536 tokens of 512 columns that all, or every
+// second one of them, read one row, join in 16 to 26 us instead of 8.2).
 // A team of lanes walks a chunk, holding one row's sum in registers; a row that lies inside the chunk is written at once, one
 // that crosses its ends leaves partial sums, which a last launch joins in order.  Rows that no token reads are zeroed beside
 // the chunks: the sort marks those that have one (looking them up in the sorted list, fifteen dependent loads, held the
@@ -20,8 +22,8 @@
 // offsets from the digit counts of all tiles (no scan launch), which a launch before it has made.  (Counts of the
 // next digit added up by the pass before, with atomics where the tokens land: 17 us a pass instead of 2.5 + 6, frequent ids
 // meet in one counter.)
-// 65 536 tokens over 19 000 rows of 512 columns in bf16, 49.6 us: two passes of count 2.7 and sort 5.1, sums 20.6 (106 MB, 5.1
-// TB/s: a large copy's rate), joins 7.2, and the starts of six launches.
+// 65 536 tokens over 19 000 rows of 512 columns in bf16, 48.5-49 us: two passes of count 3.0 and sort 6.4, sums 21.0 (106 MB, 5.0
+// TB/s: a large copy's rate), joins 8.2, and what the starts of six launches leave between them.
 #include <algorithm>
 
 #include "vec8.h"
@@ -584,7 +586,7 @@ __global__ __launch_bounds__(256) void few_tokens_kernel(Sum a, const TI* __rest
 }
 
 // ---- up to kFewRows table rows (conditions): no sort.  A team keeps one sum for each row over a chunk of tokens, and a second
-// launch adds the chunks up.  4096 tokens over three rows of 1024 columns in fp32 12.4 us (sorted 16.9): 7.7 for the sums, 4.6 for
+// launch adds the chunks up.  4096 tokens over three rows of 1024 columns in fp32 12.6 us (sorted 16.9): 8.0 for the sums, 5.2 for
 // the join; half of either is a launch's start.
 constexpr int kFewRows = 8;
 

@@ -24,7 +24,7 @@ namespace fp8 {
 constexpr int64_t kMaxBlocks = 1ll << 24;  // of 256 threads: a launch's grid holds 2^32 threads at most
 
 // Blocks of 1 x 128, row-wise only: a wave takes 512 columns of a row, 16 lanes a block, 8 elements a lane.  Bound by memory, and
-// at small sizes by the launch: 4096 x 1024 in bf16 5.5 us (2.3 TB/s).
+// at small sizes by the launch: 4096 x 19 000 in bf16 40 us (234 MB), in fp32 66 us (389 MB), 5.9 TB/s either; 4096 x 1024 6.1 us.
 template <typename T, int FMT>
 __global__ __launch_bounds__(256) void quant_rows_kernel(const T* __restrict__ x, int64_t ldx, int64_t rows, int64_t cols,
                                                          int64_t nchunk, uint8_t* __restrict__ q, int64_t ldq,
@@ -53,8 +53,8 @@ __global__ __launch_bounds__(256) void quant_rows_kernel(const T* __restrict__ x
 
 // A 128 x 128 tile read once: row-wise blocks (ROWS), blocks along the rows of the transposed operand (COLS), or both; SQ: one
 // block for the tile.  A thread holds 8 rows x 8 columns; the transposed tile goes through LDS (16-byte stores, 128 bytes a row).
-// Bound by memory: 4096 x 19 000 in bf16, both layouts, 66-69 us (311 MB: 4.6 TB/s, 0.9 of a large copy's rate); 777 x 19 001 in
-// fp32 21.6 us (89 MB: 4.1 TB/s).  Rows whose ends cut a group of eight take the edge path's clamped loads: element by element
+// Bound by memory: 4096 x 19 000 in bf16, both layouts, 66-70 us (311 MB: 4.5 TB/s, 0.9 of a large copy's rate); 777 x 19 001 in
+// fp32 23.2 us (89 MB: 3.8 TB/s).  Rows whose ends cut a group of eight take the edge path's clamped loads: element by element
 // the last column tile alone held the launch up.
 template <typename T, int FMT, bool ROWS, bool COLS, bool SQ>
 __global__ __launch_bounds__(256) void quant_tile_kernel(const T* __restrict__ x, int64_t ldx, int64_t rows, int64_t cols,

@@ -15,10 +15,10 @@
 // below a group's largest product and add the groups and the accumulator in fp32, to nearest (measured: over reductions of 512,
 // 19 200 and 70 400 1e-7, 8e-7 and 1.6e-6 of the result's norm; fp32 arithmetic 1e-7, 6e-7 and 1.3e-6).
 //
-// Bound by the matrix unit where the reduction is long: 8192 x 8192 x 8192 takes 398-411 us, 2.67-2.76 PFLOP/s (the card's
-// library: 2.69).  Short reductions are bound by their results: 4096 x 19 000 over 1024 takes 90-93 us (1.74 PFLOP/s), of which
-// the five rounds' 33 MB of stores, which all CUs make at the same time, are a third.  fp32 results: 8192 cubed 975 us (1.13
-// PFLOP/s, what the library's bf16 product reaches), 1024 x 19 000 over 4096 150 us (88 with a 16-bit result), 4096 x 19 000
+// Bound by the matrix unit where the reduction is long: 8192 x 8192 x 8192 takes 416 us, 2.64 PFLOP/s (the card's
+// library: 2.69), in an unbroken row of twenty 480, where the clock gives way; the matrix unit is busy 0.70 of the time.  Short reductions are bound by their results: 4096 x 19 000 over 1024 takes 90-93 us (1.74 PFLOP/s), of which
+// the five rounds' 33 MB of stores, which all CUs make at the same time, are a third.  fp32 results: 8192 cubed 960-975 us (1.13
+// PFLOP/s; the library's bf16 product 1.22; matrix unit busy 0.61), 1024 x 19 000 over 4096 150 us (88 with a 16-bit result), 4096 x 19 000
 // over 1024 183.
 #include <algorithm>
 
@@ -402,7 +402,7 @@ __global__ __launch_bounds__(64 * WM * WN, WPE) void gemm_fp8_kernel(Args a, int
 #endif
 }
 
-// 4096 x 1024 in two parts: 15 us (the 34 MB that the product just wrote at 2.8 TB/s); 128 x 256 in 50: 2.9 us.
+// 4096 x 1024 in four parts: 14.4 us (the 67 MB that the product just wrote); 128 x 256 in 50: 4.0 us.
 // Y = alpha * sum of the slabs + bias: four columns a thread, SG threads share their slabs (SG > 1 where the result alone is
 // too small to keep the chip busy) and meet in LDS, in a fixed order.
 template <typename TY, int SG>

@@ -1,7 +1,8 @@
 """Tensor-level wrappers over the C-ABI (one function per entry point of include/c2mi.h).
 
 All tensors live on the GPU; shapes/strides are checked here on the host before any
-kernel is enqueued.  Nothing in this module computes on the CPU.
+kernel is enqueued.  Nothing in this module computes on the CPU, and nothing records an
+autograd graph: gradients come from the functions that compute them.
 """
 import os
 from contextlib import nullcontext
