@@ -438,8 +438,9 @@ __global__ __launch_bounds__(256) void join_slabs_kernel(const float* __restrict
         if (n + c < N) st_from_f32<TY>(Y + m * ldy + n + c, alpha * s[c] + (bias ? bias[n + c] : 0.f));
 }
 
-// ---- how a product is cut (fp32 results: wide): tiles of 256 x 256 or 128 x 128 (wide: these only), the reduction in `splits` parts where the tiles alone leave CUs
-// idle; or 256 x 256 tiles for the columns that make whole rounds of the chip, and the best cut for the rest.
+// ---- how a product is cut: tiles of 256 x 256 or 128 x 128, the reduction in `splits` parts where the tiles alone leave CUs idle; or
+// 256 x 256 tiles for the columns that make whole rounds of the chip, and the best cut for the rest.  Wide (fp32 results): 128 x 128
+// tiles, in parts or not.
 struct Cut {
     int big, splits, kb_per_split;
     int64_t lds, slab;
