@@ -542,7 +542,8 @@ extern "C" int c2_distill_topk_fwd_bwd(const void* logits, int l_dtype, int64_t 
     C2_CHECK(idx_bytes == 4 || idx_bytes == 8, "idx_bytes: 4 (int32) or 8 (int64)");
     C2_CHECK(temperature > 0.f && temperature < INFINITY, "temperature must be positive and finite");
     // (its square scales the loss, log2(e) / T the exponents: below, the one loses its bits and the other is infinite)
-    C2_CHECK(temperature * temperature >= 1.17549435e-38f && temperature * temperature < INFINITY, "temperature: its square must be a normal fp32 number");
+    C2_CHECK(temperature * temperature >= 1.17549435e-38f && temperature * temperature < INFINITY,
+             "temperature: its square must be a normal fp32 number");
     C2_CHECK(B > 0 && V > 0 || loss_add, "an empty batch has no loss to set: clear it and add");
     if (B == 0 || V == 0) return 0;
     C2_CHECK(logits && loss_out && ws && ldl >= V && (!dlogits || lddl >= V), "bad arguments");

@@ -15,11 +15,11 @@
 // below a group's largest product and add the groups and the accumulator in fp32, to nearest (measured: over reductions of 512,
 // 19 200 and 70 400 1e-7, 8e-7 and 1.6e-6 of the result's norm; fp32 arithmetic 1e-7, 6e-7 and 1.3e-6).
 //
-// Bound by the matrix unit where the reduction is long: 8192 x 8192 x 8192 takes 416 us, 2.64 PFLOP/s (the card's
-// library: 2.69), in an unbroken row of twenty 480, where the clock gives way; the matrix unit is busy 0.70 of the time.  Short reductions are bound by their results: 4096 x 19 000 over 1024 takes 90-93 us (1.74 PFLOP/s), of which
-// the five rounds' 33 MB of stores, which all CUs make at the same time, are a third.  fp32 results: 8192 cubed 960-975 us (1.13
-// PFLOP/s; the library's bf16 product 1.22; matrix unit busy 0.61), 1024 x 19 000 over 4096 150 us (88 with a 16-bit result), 4096 x 19 000
-// over 1024 183.
+// Bound by the matrix unit where the reduction is long: 8192 x 8192 x 8192 takes 416 us, 2.64 PFLOP/s (the card's library: 2.69),
+// in an unbroken row of twenty 480, where the clock gives way; the matrix unit is busy 0.70 of the time.  Short reductions are
+// bound by their results: 4096 x 19 000 over 1024 takes 90-93 us (1.74 PFLOP/s), of which the five rounds' 33 MB of stores, which
+// all CUs make at the same time, are a third.  fp32 results: 8192 cubed 960-975 us (1.13 PFLOP/s; the library's bf16 product
+// 1.22; matrix unit busy 0.61), 1024 x 19 000 over 4096 150 us (88 with a 16-bit result), 4096 x 19 000 over 1024 183.
 #include <algorithm>
 
 #include "fp8.h"
